@@ -107,6 +107,11 @@ std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
   return {rows, rows.size(0) <= 1 ? rows.size(1) : rows.stride(0)};
 }
 
+// The operators have no forward-mode derivative; outputs made without one would lose it.
+void refuse_tangent(const char* what, const Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 bool needs_gradient(std::initializer_list<const Tensor*> tensors) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : tensors)
@@ -170,6 +175,7 @@ struct Embedding : Function<Embedding> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool graph = at::GradMode::is_enabled();
     torch::NoGradGuard no_grad;
+    refuse_tangent("token_embedding", grads[0]);
     const Tensor ids = ctx->get_saved_variables()[0];
     const auto shape = ctx->saved_data["shape"].toTuple();
     const int64_t vocab = shape->elements()[0].toInt(), dim = shape->elements()[1].toInt();
@@ -190,6 +196,7 @@ struct Embedding : Function<Embedding> {
 };
 
 Tensor embedding(const Tensor& table, const Tensor& ids, double scale, int64_t padding) {
+  refuse_tangent("token_embedding", table);
   const Tensor flat = ids.dim() == 1 && ids.is_contiguous() ? ids : ids.reshape({-1}).contiguous();
   const Tensor out = needs_gradient({&table}) ? Embedding::apply(table, flat, scale, padding)
                                               : lookup(table, flat, scale, padding);
@@ -272,6 +279,7 @@ struct Dispatch : Function<Dispatch> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool graph = at::GradMode::is_enabled();
     torch::NoGradGuard no_grad;
+    refuse_tangent("dispatch_to_experts", grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     return once({gather(grads[0], Tensor(), saved[0], saved[1]), Tensor(), Tensor()}, graph);
   }
@@ -286,6 +294,7 @@ struct Combine : Function<Combine> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool graph = at::GradMode::is_enabled();
     torch::NoGradGuard no_grad;
+    refuse_tangent("combine_from_experts", grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     const auto [grad, grad_stride] = rows_of(grads[0]);
     const auto [rows, rows_stride] = rows_of(saved[0]);
@@ -309,9 +318,12 @@ struct Combine : Function<Combine> {
 };
 
 Tensor dispatch(const Tensor& x, const Tensor& offsets, const Tensor& position) {
+  refuse_tangent("dispatch_to_experts", x);
   return needs_gradient({&x}) ? Dispatch::apply(x, offsets, position) : spread(x, offsets, position);
 }
 Tensor combine(const Tensor& rows, const Tensor& given, const Tensor& offsets, const Tensor& position) {
+  refuse_tangent("combine_from_experts", rows);
+  refuse_tangent("combine_from_experts", given);
   const Tensor weights = given.contiguous();
   return needs_gradient({&rows, &weights}) ? Combine::apply(rows, weights, offsets, position)
                                            : gather(rows, weights, offsets, position);
@@ -376,6 +388,7 @@ struct LinearCrossEntropy : Function<LinearCrossEntropy> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool graph = at::GradMode::is_enabled();
     torch::NoGradGuard no_grad;
+    refuse_tangent("linear_cross_entropy", grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     const auto options = ctx->saved_data["call"].toTuple();
     const int64_t ignore = options->elements()[0].toInt(), reduction = options->elements()[1].toInt();
@@ -402,6 +415,8 @@ struct LinearCrossEntropy : Function<LinearCrossEntropy> {
 
 Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& given,
                             int64_t ignore, int64_t reduction) {
+  refuse_tangent("linear_cross_entropy", hidden);
+  refuse_tangent("linear_cross_entropy", weight);
   const Tensor targets = given.contiguous();
   if (needs_gradient({&hidden, &weight}))
     return LinearCrossEntropy::apply(hidden, weight, targets, ignore, reduction);
@@ -413,9 +428,12 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
 // Every tensor's elements fill a range of memory, outs[i] in tensors[i]'s order.
 Tensor gradients(const std::vector<Tensor>& tensors, const std::vector<Tensor>& outs, bool clip,
                  double max_norm, double eps) {
+  const char* what = clip ? "clip_gradients" : "gradient_norm";
   std::vector<PurinGradient> list(tensors.size());
   bool wide = false;
   for (size_t i = 0; i < tensors.size(); ++i) {
+    refuse_tangent(what, tensors[i]);
+    if (clip) refuse_tangent(what, outs[i]);
     list[i] = {tensors[i].data_ptr(), outs[i].data_ptr(), tensors[i].numel(),
                code_of(tensors[i].scalar_type()), 0};
     wide |= list[i].dtype == PURIN_OPS_FLOAT64;

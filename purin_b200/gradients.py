@@ -44,7 +44,8 @@ def gradient_norm(tensors):
     """
     tensors = _tensors("gradient_norm", tensors)
     if not all(map(_dense, tensors)):
-        tensors = [t if _dense(t) else t.detach().contiguous() for t in tensors]
+        with torch.no_grad():
+            tensors = [t if _dense(t) else t.contiguous() for t in tensors]
     return _ops.load().gradients(tensors, tensors, False, 0.0, 0.0)
 
 
