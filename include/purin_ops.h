@@ -83,7 +83,8 @@ int32_t purin_route(const PurinRouteArgs* args, void* workspace, size_t workspac
                     void* stream);
 
 /* Rows moved by a routing.  Token rows are (tokens, dim), sorted rows
- * (tokens * slots, dim); a sorted row r is dropped if r >= offsets[num_experts].
+ * (tokens * slots, dim); a sorted row r is dropped if r >= offsets[num_experts].  A
+ * position outside [0, tokens * slots) is neither read nor written.
  *   spread: sorted[position[t,k]] = token_rows[t], dropped rows zero
  *   gather: token_out[t] = sum over kept k of weights[t,k] * sorted_rows[position[t,k]]
  *           (weights null: 1), summed in 32 bits (64 for double), k ascending

@@ -9,6 +9,9 @@
 // ones last), so all of them go by the token: a token's row is read once and its slots'
 // rows are written, or the other way round, with no atomics, no fill and no count on the
 // host.  Bound by HBM: tokens x slots x dim elements one way, tokens x dim the other.
+//
+// The routing is the caller's: a position outside [0, tokens x slots), which purin_route does
+// not make, is neither read nor written; its slot counts as dropped.
 #include "ops_sort.cuh"
 
 namespace purin {
@@ -25,12 +28,18 @@ constexpr int kThreads = 256;
 template <int V>
 constexpr int kPacksAtOnce = V == 1 ? 4 : 1;
 
+// Sorted rows in use, at most all of them.
+__device__ __forceinline__ int32_t kept_of(const int32_t* kept_rows, int32_t rows) {
+  return max(0, min(*kept_rows, rows));
+}
+__device__ __forceinline__ bool below(int32_t r, int32_t end) { return uint32_t(r) < uint32_t(end); }
+
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads)
 spread_kernel(const int32_t* position, const int32_t* kept_rows, int64_t tokens, int slots,
               int64_t packs, const T* x, int64_t stride, T* out) {
   constexpr int C = kPacksAtOnce<V>;
-  const int32_t kept = *kept_rows;
+  const int32_t rows = int32_t(tokens * slots), kept = kept_of(kept_rows, rows);
   const int64_t items = (packs + C - 1) / C, total = tokens * items;
   const bool fits32 = total <= INT32_MAX;
   for (int64_t at = int64_t(blockIdx.x) * kThreads + threadIdx.x; at < total;
@@ -43,12 +52,19 @@ spread_kernel(const int32_t* position, const int32_t* kept_rows, int64_t tokens,
       if (C == 1 || c + j * items < packs) p[j] = *reinterpret_cast<const Pack<T, V>*>(x + t * stride + (c + j * items) * V);
 #pragma unroll
     for (int i = 0; i < V; ++i) zero.v[i] = narrow<T>(acc_t<T>(0));
-    for (int k = 0; k < slots; ++k) {
-      const int64_t r = position[t * slots + k];
-      Pack<T, V>* to = reinterpret_cast<Pack<T, V>*>(out) + r * packs + c;
+    constexpr int kAhead = 4;  // positions loaded at a time
+    for (int first = 0; first < slots; first += kAhead) {
+      int32_t r[kAhead];
 #pragma unroll
-      for (int j = 0; j < C; ++j)
-        if (C == 1 || c + j * items < packs) to[j * items] = r < kept ? p[j] : zero;
+      for (int k = 0; k < kAhead; ++k) r[k] = first + k < slots ? position[t * slots + first + k] : -1;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (!below(r[k], rows)) continue;
+        Pack<T, V>* to = reinterpret_cast<Pack<T, V>*>(out) + r[k] * packs + c;
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (C == 1 || c + j * items < packs) to[j * items] = r[k] < kept ? p[j] : zero;
+      }
     }
   }
 }
@@ -59,7 +75,7 @@ gather_kernel(const int32_t* position, const int32_t* kept_rows, int64_t tokens,
               int64_t packs, const T* rows, int64_t stride, const W* weights, T* out) {
   using A = acc_t<T>;
   constexpr int C = kPacksAtOnce<V>;
-  const int32_t kept = *kept_rows;
+  const int32_t kept = kept_of(kept_rows, int32_t(tokens * slots));
   const int64_t items = (packs + C - 1) / C, total = tokens * items;
   const bool fits32 = total <= INT32_MAX;
   for (int64_t at = int64_t(blockIdx.x) * kThreads + threadIdx.x; at < total;
@@ -77,16 +93,16 @@ gather_kernel(const int32_t* position, const int32_t* kept_rows, int64_t tokens,
       Pack<T, V> p[kAhead][C];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        r[k] = first + k < slots ? position[t * slots + first + k] : kept;
+        r[k] = first + k < slots ? position[t * slots + first + k] : -1;
         // A dropped slot's row and weight may hold anything: they are not read.
 #pragma unroll
         for (int j = 0; j < C; ++j)
-          if (r[k] < kept && (C == 1 || c + j * items < packs))
+          if (below(r[k], kept) && (C == 1 || c + j * items < packs))
             p[k][j] = *reinterpret_cast<const Pack<T, V>*>(rows + r[k] * stride + (c + j * items) * V);
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        if (r[k] >= kept) continue;
+        if (!below(r[k], kept)) continue;
         const A w = kWeighted ? A(weights[t * slots + first + k]) : A(1);
 #pragma unroll
         for (int j = 0; j < C; ++j)
@@ -121,7 +137,7 @@ combine_backward_kernel(const int32_t* position, const int32_t* kept_rows, int64
   using A = acc_t<T>;
   constexpr int kTokens = kThreads / G, kWarps = G / 32, C = kPacksAtOnce<V>;
   __shared__ A part[kThreads / 32][kSlotsAtOnce];
-  const int32_t kept = *kept_rows;
+  const int32_t all = int32_t(tokens * slots), kept = kept_of(kept_rows, all);
   const int lane = threadIdx.x & 31, in = threadIdx.x % G, warp = threadIdx.x >> 5;
   for (int64_t t0 = int64_t(blockIdx.x) * kTokens; t0 < tokens; t0 += int64_t(gridDim.x) * kTokens) {
     const int64_t t = t0 + threadIdx.x / G;
@@ -132,6 +148,7 @@ combine_backward_kernel(const int32_t* position, const int32_t* kept_rows, int64
 #pragma unroll
       for (int k = 0; k < kSlotsAtOnce; ++k) {
         r[k] = real_token && first + k < slots ? position[t * slots + first + k] : -1;
+        if (r[k] >= all) r[k] = -1;
         dot[k] = A(0);
       }
       for (int64_t c = in; real_token && c < packs; c += G * C) {
@@ -179,7 +196,7 @@ combine_backward_kernel(const int32_t* position, const int32_t* kept_rows, int64
 #pragma unroll
           for (int d = 16; d; d >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], d);
           if constexpr (kWarps == 1) {
-            if (lane == 0 && r[k] >= 0) grad_weights[t * slots + first + k] = W(dot[k]);
+            if (lane == 0 && real_token && first + k < slots) grad_weights[t * slots + first + k] = W(dot[k]);
           } else {
             if (lane == 0) part[warp][k] = dot[k];
           }

@@ -24,7 +24,8 @@ class ExpertRouting(NamedTuple):
 
     ``offsets[e]:offsets[e + 1]`` are expert e's sorted rows; ``position[t, k]`` is the
     sorted row of slot k of token t; ``source[r]`` is the slot ``t * slots + k`` of sorted
-    row r.  Rows from ``offsets[-1]`` on belong to dropped slots.
+    row r.  Rows from ``offsets[-1]`` on belong to dropped slots.  A routing is used as
+    ``route_to_experts`` made it, whole: a part of its tokens is routed anew.
     """
 
     offsets: torch.Tensor
@@ -52,6 +53,23 @@ def route_to_experts(experts, num_experts) -> ExpertRouting:
     return ExpertRouting(*_ops.load().route(experts, num_experts))
 
 
+def _check_routing(what, x, routing):
+    """``x`` and the routing are on one CUDA device, and the routing is whole."""
+    offsets, position, source = routing
+    _ops.require_cuda(what, x, position, offsets)
+    if position.dim() != 2 or position.shape[1] < 1 or offsets.dim() != 1 or offsets.shape[0] < 2:
+        raise ValueError(f"{what}: the routing's position must have shape (tokens, slots) and offsets "
+                         f"(experts + 1,), got {tuple(position.shape)} and {tuple(offsets.shape)}")
+    for name, t in (("position", position), ("offsets", offsets)):
+        if t.dtype != torch.int32:
+            raise TypeError(f"{what}: the routing's {name} must be int32, got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: the routing's {name} must be contiguous; route_to_experts makes it so")
+    # Positions name rows of the whole routing: of a part of it, rows that are not there.
+    if isinstance(source, torch.Tensor) and source.numel() != position.numel():
+        raise ValueError(f"{what}: the routing has {source.numel()} slots but {position.numel()} positions")
+
+
 def _check_rows(what, name, t, rows):
     if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
         raise ValueError(f"{what}: {name} must have shape ({rows}, dim), got {tuple(t.shape)}")
@@ -64,7 +82,7 @@ def dispatch_to_experts(x, routing: ExpertRouting):
     Differentiable: a token's gradient is the sum of its kept slots' gradients.
     """
     what = "dispatch_to_experts"
-    _ops.require_cuda(what, x, routing.position)
+    _check_routing(what, x, routing)
     _check_rows(what, "x", x, routing.position.shape[0])
     return _ops.load().dispatch(x, routing.offsets, routing.position)
 
@@ -78,7 +96,8 @@ def combine_from_experts(rows, weights, routing: ExpertRouting):
     float64 rows).
     """
     what = "combine_from_experts"
-    _ops.require_cuda(what, rows, weights, routing.position)
+    _check_routing(what, rows, routing)
+    _ops.require_cuda(what, rows, weights)
     tokens, slots = routing.position.shape
     _check_rows(what, "rows", rows, tokens * slots)
     if weights.shape != (tokens, slots):

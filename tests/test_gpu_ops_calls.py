@@ -67,3 +67,58 @@ def test_forward_mode_tangents_of_gradients_are_not_lost():
         with pytest.raises(RuntimeError, match="forward-mode"):
             clip_gradients([t.clone()], 1.0, out=[dual])
     assert bool((t == 1).all())
+
+
+@pytest.mark.parametrize("dim", [5, 72, 130, 1031])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_positions_outside_the_rows_are_neither_read_nor_written(dtype, dim):
+    """A routing made by hand: such slots are dropped, and the memory around keeps its values."""
+    tokens, slots, far = 6, 3, 2 ** 31 - 1
+    routing = route_to_experts(torch.arange(18, device=DEV).view(6, 3) % 5, 5)
+    position = routing.position.clone()
+    bad = torch.zeros(6, 3, dtype=torch.bool, device=DEV)
+    for at, value in (((0, 0), 18), ((1, 2), far), ((2, 1), -1), ((5, 2), -far - 1), ((4, 0), 19)):
+        position[at] = value
+        bad[at] = True
+    offsets = routing.offsets.clone()
+    offsets[-1] = 1000  # more rows than there are
+    made = routing._replace(position=position, offsets=offsets)
+    g = torch.Generator(device=DEV).manual_seed(dim)
+    x = torch.randn(tokens, dim, generator=g, device=DEV).to(dtype).requires_grad_()
+    rows = torch.randn(18, dim, generator=g, device=DEV).to(dtype).requires_grad_()
+    weights = torch.rand(tokens, slots, generator=g, device=DEV).requires_grad_()
+    kept = ~bad
+    at = torch.where(kept, position, 0).long()
+    sent = dispatch_to_experts(x, made)
+    assert torch.equal(sent[position[kept].long()], x[kept.nonzero()[:, 0]])
+    picked = torch.where(kept[:, :, None], rows.detach().double()[at], 0.0)
+    out = combine_from_experts(rows, weights, made)
+    want = (picked * weights.detach().double()[:, :, None]).sum(1)
+    limit = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -20
+    assert (out.double() - want).abs().max() <= limit * (1 + want.abs().max())
+    grad = torch.randn(tokens, dim, generator=g, device=DEV).to(dtype)
+    drows, dweights = torch.autograd.grad(out, (rows, weights), grad)
+    want = (picked * grad.double()[:, None, :]).sum(2)
+    assert (dweights.double() - want).abs().max() <= 2.0 ** -16 * (1 + want.abs().max())
+    assert bool((dweights[bad] == 0).all())
+    want = (grad.double()[:, None, :] * weights.detach().double()[:, :, None])[kept]
+    assert (drows.double()[position[kept].long()] - want).abs().max() <= limit * (1 + want.abs().max())
+    back = torch.randn(18, dim, generator=g, device=DEV).to(dtype)
+    dx, = torch.autograd.grad(sent, x, back)
+    want = torch.where(kept[:, :, None], back.double()[at], 0.0).sum(1)
+    assert (dx.double() - want).abs().max() <= limit * (1 + want.abs().max())
+
+
+def test_routings_that_are_not_whole_are_refused():
+    routing = route_to_experts(torch.arange(18, device=DEV).view(6, 3) % 5, 5)
+    x, rows, weights = torch.ones(6, 8, device=DEV), torch.ones(18, 8, device=DEV), torch.ones(6, 3, device=DEV)
+    cases = [(ValueError, dict(position=routing.position[:, :1])), (ValueError, dict(position=routing.position[:2])),
+             (ValueError, dict(offsets=routing.offsets.cpu())), (ValueError, dict(offsets=routing.offsets[::2])),
+             (ValueError, dict(position=routing.position.cpu())), (TypeError, dict(position=routing.position.long()))]
+    for error, change in cases:
+        made = routing._replace(**change)
+        tokens, slots = made.position.shape
+        with pytest.raises(error):
+            dispatch_to_experts(x[:tokens], made)
+        with pytest.raises(error):
+            combine_from_experts(rows[:tokens * slots], weights[:tokens, :slots], made)
