@@ -119,22 +119,24 @@ bool needs_gradient(std::initializer_list<const Tensor*> tensors) {
   return false;
 }
 
-// The gradients of a node that is differentiable once: asked for with create_graph, they
-// carry a node that raises when it is differentiated.
-variable_list once(variable_list grads, bool graph) {
-  if (!graph) return grads;
+// The same values, with a node that raises when it is differentiated.
+variable_list raising(variable_list values, const char* message) {
   variable_list defined;
-  for (const Variable& g : grads)
-    if (g.defined()) defined.push_back(g.detach().requires_grad_());
-  if (defined.empty()) return grads;
-  auto node = std::make_shared<torch::autograd::DelayedError>(
-      "this operator's gradient is not differentiable", int64_t(defined.size()));
+  for (const Variable& v : values)
+    if (v.defined()) defined.push_back(v.detach().requires_grad_());
+  if (defined.empty()) return values;
+  auto node = std::make_shared<torch::autograd::DelayedError>(message, int64_t(defined.size()));
   at::AutoGradMode enabled(true);
   variable_list wrapped = (*node)(std::move(defined));
   size_t at = 0;
-  for (Variable& g : grads)
-    if (g.defined()) g = wrapped[at++];
-  return grads;
+  for (Variable& v : values)
+    if (v.defined()) v = wrapped[at++];
+  return values;
+}
+
+// The gradients of a node that is differentiable once, which create_graph may ask for.
+variable_list once(variable_list grads, bool graph) {
+  return graph ? raising(std::move(grads), "this operator's gradient is not differentiable") : grads;
 }
 
 // ---- embedding -----------------------------------------------------------------------
@@ -430,13 +432,14 @@ Tensor gradients(const std::vector<Tensor>& tensors, const std::vector<Tensor>& 
                  double max_norm, double eps) {
   const char* what = clip ? "clip_gradients" : "gradient_norm";
   std::vector<PurinGradient> list(tensors.size());
-  bool wide = false;
+  bool wide = false, graph = false;
   for (size_t i = 0; i < tensors.size(); ++i) {
     refuse_tangent(what, tensors[i]);
     if (clip) refuse_tangent(what, outs[i]);
     list[i] = {tensors[i].data_ptr(), outs[i].data_ptr(), tensors[i].numel(),
                code_of(tensors[i].scalar_type()), 0};
     wide |= list[i].dtype == PURIN_OPS_FLOAT64;
+    graph |= tensors[i].requires_grad();
   }
   Tensor norm = at::empty({}, tensors[0].options().dtype(wide ? at::kDouble : at::kFloat));
   PurinGradientsArgs a = {};
@@ -454,6 +457,8 @@ Tensor gradients(const std::vector<Tensor>& tensors, const std::vector<Tensor>& 
   call("purin_gradients", a.device, [&](void* s) { return purin_gradients(&a, pointer(ws), bytes_of(ws), s); });
   if (clip)  // autograd learns of what was written in place
     for (const Tensor& o : outs) o.unsafeGetTensorImpl()->bump_version();
+  else if (graph && at::GradMode::is_enabled())
+    return raising({norm}, "gradient_norm is not differentiable")[0];
   return norm;
 }
 

@@ -40,12 +40,12 @@ def _dense(t):
 def gradient_norm(tensors):
     """``sqrt(sum of x^2)`` over all elements of ``tensors``, a 0-d tensor on their device.
 
-    float32, or float64 if one of the tensors is; partial sums are joined in float64.
+    float32, or float64 if one of the tensors is; partial sums are joined in float64.  Not
+    differentiable: the norm of tensors that need a gradient raises in a backward.
     """
     tensors = _tensors("gradient_norm", tensors)
     if not all(map(_dense, tensors)):
-        with torch.no_grad():
-            tensors = [t if _dense(t) else t.contiguous() for t in tensors]
+        tensors = [t if _dense(t) else t.contiguous() for t in tensors]
     return _ops.load().gradients(tensors, tensors, False, 0.0, 0.0)
 
 
@@ -53,7 +53,7 @@ def clip_gradients(tensors, max_norm, *, out=None, eps=1e-6):
     """Scale ``tensors`` by ``min(1, max_norm / (norm + eps))``; returns the norm.
 
     In place, or into ``out`` (tensors of the same shapes and types); no output may share
-    memory with another tensor.  The norm is that before clipping; if it is NaN or infinite,
+    memory with another tensor.  Autograd records neither the scaling nor the norm.  The norm is that before clipping; if it is NaN or infinite,
     so are clipped values: ask ``isfinite`` of the norm to skip a step.
     """
     what = "clip_gradients"

@@ -69,6 +69,20 @@ def test_forward_mode_tangents_of_gradients_are_not_lost():
     assert bool((t == 1).all())
 
 
+def test_norm_of_tensors_with_a_graph_raises_when_differentiated():
+    x = torch.arange(6.0, device=DEV).view(2, 3).requires_grad_()
+    y = x * x
+    want = float(y.detach().double().square().sum().sqrt())
+    for of in (lambda t: t, lambda t: t[:, ::2]):
+        norm = gradient_norm([of(y), torch.zeros(3, device=DEV)])
+        with pytest.raises(RuntimeError, match="gradient_norm is not differentiable"):
+            norm.backward()
+    assert abs(gradient_norm(y).item() - want) <= 1e-6 * want
+    with torch.no_grad():
+        assert not gradient_norm(y).requires_grad
+    assert not gradient_norm(y.detach()).requires_grad
+
+
 @pytest.mark.parametrize("dim", [5, 72, 130, 1031])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_positions_outside_the_rows_are_neither_read_nor_written(dtype, dim):
