@@ -2,10 +2,13 @@
 // and workspaces in C++.  A training step calls these operators many times with little work
 // in each; the nodes' host time in Python (16 us forward, 25 us backward) was most of such a
 // call.  Arguments are checked by the Python modules that call this one.
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
 #include <nvtx3/nvToolsExt.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <atomic>
@@ -107,6 +110,17 @@ std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
   return {rows, rows.size(0) <= 1 ? rows.size(1) : rows.stride(0)};
 }
 
+// A tracer sees the outputs' allocation and not what is written to them by pointer: the traced
+// function would return memory that nobody wrote.
+void refuse_tracing(const char* what) {
+  using c10::impl::TorchDispatchModeTLS;
+  const bool traced = torch::jit::tracer::isTracing() ||
+                      c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+                      (TorchDispatchModeTLS::any_modes_set() &&
+                       TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
+  TORCH_CHECK(!traced, what, " cannot be traced");
+}
+
 // The operators have no forward-mode derivative; outputs made without one would lose it.
 void refuse_tangent(const char* what, const Tensor& t) {
   TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivative");
@@ -177,6 +191,7 @@ struct Embedding : Function<Embedding> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool graph = at::GradMode::is_enabled();
     torch::NoGradGuard no_grad;
+    refuse_tracing("token_embedding");
     refuse_tangent("token_embedding", grads[0]);
     const Tensor ids = ctx->get_saved_variables()[0];
     const auto shape = ctx->saved_data["shape"].toTuple();
@@ -198,6 +213,7 @@ struct Embedding : Function<Embedding> {
 };
 
 Tensor embedding(const Tensor& table, const Tensor& ids, double scale, int64_t padding) {
+  refuse_tracing("token_embedding");
   refuse_tangent("token_embedding", table);
   const Tensor flat = ids.dim() == 1 && ids.is_contiguous() ? ids : ids.reshape({-1}).contiguous();
   const Tensor out = needs_gradient({&table}) ? Embedding::apply(table, flat, scale, padding)
@@ -211,6 +227,7 @@ Tensor embedding(const Tensor& table, const Tensor& ids, double scale, int64_t p
 // ---- routing -------------------------------------------------------------------------
 
 std::tuple<Tensor, Tensor, Tensor> route(const Tensor& given, int64_t num_experts) {
+  refuse_tracing("route_to_experts");
   const Tensor experts = given.contiguous();
   const auto options = experts.options().dtype(at::kInt);
   Tensor offsets = at::empty({num_experts + 1}, options);
@@ -281,6 +298,7 @@ struct Dispatch : Function<Dispatch> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool graph = at::GradMode::is_enabled();
     torch::NoGradGuard no_grad;
+    refuse_tracing("dispatch_to_experts");
     refuse_tangent("dispatch_to_experts", grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     return once({gather(grads[0], Tensor(), saved[0], saved[1]), Tensor(), Tensor()}, graph);
@@ -296,6 +314,7 @@ struct Combine : Function<Combine> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool graph = at::GradMode::is_enabled();
     torch::NoGradGuard no_grad;
+    refuse_tracing("combine_from_experts");
     refuse_tangent("combine_from_experts", grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     const auto [grad, grad_stride] = rows_of(grads[0]);
@@ -320,10 +339,12 @@ struct Combine : Function<Combine> {
 };
 
 Tensor dispatch(const Tensor& x, const Tensor& offsets, const Tensor& position) {
+  refuse_tracing("dispatch_to_experts");
   refuse_tangent("dispatch_to_experts", x);
   return needs_gradient({&x}) ? Dispatch::apply(x, offsets, position) : spread(x, offsets, position);
 }
 Tensor combine(const Tensor& rows, const Tensor& given, const Tensor& offsets, const Tensor& position) {
+  refuse_tracing("combine_from_experts");
   refuse_tangent("combine_from_experts", rows);
   refuse_tangent("combine_from_experts", given);
   const Tensor weights = given.contiguous();
@@ -390,6 +411,7 @@ struct LinearCrossEntropy : Function<LinearCrossEntropy> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool graph = at::GradMode::is_enabled();
     torch::NoGradGuard no_grad;
+    refuse_tracing("linear_cross_entropy");
     refuse_tangent("linear_cross_entropy", grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     const auto options = ctx->saved_data["call"].toTuple();
@@ -417,6 +439,7 @@ struct LinearCrossEntropy : Function<LinearCrossEntropy> {
 
 Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& given,
                             int64_t ignore, int64_t reduction) {
+  refuse_tracing("linear_cross_entropy");
   refuse_tangent("linear_cross_entropy", hidden);
   refuse_tangent("linear_cross_entropy", weight);
   const Tensor targets = given.contiguous();
@@ -431,6 +454,7 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
 Tensor gradients(const std::vector<Tensor>& tensors, const std::vector<Tensor>& outs, bool clip,
                  double max_norm, double eps) {
   const char* what = clip ? "clip_gradients" : "gradient_norm";
+  refuse_tracing(what);
   std::vector<PurinGradient> list(tensors.size());
   bool wide = false, graph = false;
   for (size_t i = 0; i < tensors.size(); ++i) {

@@ -83,6 +83,44 @@ def test_norm_of_tensors_with_a_graph_raises_when_differentiated():
     assert not gradient_norm(y.detach()).requires_grad
 
 
+@pytest.mark.parametrize("index", range(6))
+@pytest.mark.parametrize("tracer", ["make_fx", "make_fx before dispatch", "jit"])
+def test_operators_are_not_traced_as_empty_memory(index, tracer):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    _, run, t = operators()[index]
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        if tracer == "jit":
+            torch.jit.trace(run, t, check_trace=False)
+        else:
+            make_fx(run, pre_dispatch="before" in tracer)(t)
+    run(t)
+
+
+def test_gradients_and_routes_are_not_traced_as_empty_memory():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    t = torch.ones(9, device=DEV)
+    for run in (lambda v: gradient_norm([v]), lambda v: clip_gradients([v], 1.0),
+                lambda v: route_to_experts((v > 0).int().view(9, 1), 2)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(run)(t)
+    assert bool((t == 1).all())
+
+
+def test_other_dispatch_modes_see_the_operators_run():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Passing(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    for _, run, t in operators():
+        with Passing():
+            got = run(t)
+        assert torch.equal(got, run(t))
+
+
 @pytest.mark.parametrize("dim", [5, 72, 130, 1031])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_positions_outside_the_rows_are_neither_read_nor_written(dtype, dim):
