@@ -2,6 +2,7 @@
 // and workspaces in C++.  A training step calls these operators many times with little work
 // in each; the nodes' host time in Python (16 us forward, 25 us backward) was most of such a
 // call.  Arguments are checked by the Python modules that call this one.
+#include <c10/core/InferenceMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
@@ -459,7 +460,12 @@ Tensor gradients(const std::vector<Tensor>& tensors, const std::vector<Tensor>& 
   bool wide = false, graph = false;
   for (size_t i = 0; i < tensors.size(); ++i) {
     refuse_tangent(what, tensors[i]);
-    if (clip) refuse_tangent(what, outs[i]);
+    if (clip) {
+      refuse_tangent(what, outs[i]);
+      // Counting the change below would raise, behind a launch that has written.
+      TORCH_CHECK(!outs[i].is_inference() || c10::InferenceMode::is_enabled(), what,
+                  ": a tensor of inference mode is not written outside it");
+    }
     list[i] = {tensors[i].data_ptr(), outs[i].data_ptr(), tensors[i].numel(),
                code_of(tensors[i].scalar_type()), 0};
     wide |= list[i].dtype == PURIN_OPS_FLOAT64;

@@ -121,6 +121,18 @@ def test_other_dispatch_modes_see_the_operators_run():
         assert torch.equal(got, run(t))
 
 
+def test_clipping_does_not_write_what_it_refuses():
+    """Tensors of inference mode are not written outside it."""
+    with torch.inference_mode():
+        t = torch.full((1000,), 2.0, device=DEV)
+    with pytest.raises(RuntimeError, match="nference"):
+        clip_gradients([t], 1.0)
+    assert bool((t == 2).all())
+    with torch.inference_mode():
+        clip_gradients([t], 1.0)
+    assert abs(float(t.double().norm()) - 1.0) < 1e-5
+
+
 @pytest.mark.parametrize("dim", [5, 72, 130, 1031])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_positions_outside_the_rows_are_neither_read_nor_written(dtype, dim):
