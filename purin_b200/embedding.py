@@ -7,6 +7,8 @@ order, in 32 bits (64 for float64), so it is the same from run to run.
 
 from __future__ import annotations
 
+import torch
+
 from purin_b200 import _native_ops as _ops
 
 _WHAT = "token_embedding"
@@ -26,5 +28,7 @@ def token_embedding(table, ids, *, scale=1.0, padding_index=None):
     _ops.require_whole(_WHAT, "ids", ids)
     if padding_index is not None and not 0 <= int(padding_index) < table.shape[0]:
         raise ValueError(f"{_WHAT}: padding_index must be a row of the table")
+    if isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
+        raise TypeError(f"{_WHAT}: scale must be a number, got a tensor that needs a gradient")
     return _ops.load().embedding(table, ids, float(scale),
                                  -1 if padding_index is None else int(padding_index))

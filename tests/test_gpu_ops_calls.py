@@ -133,6 +133,16 @@ def test_clipping_does_not_write_what_it_refuses():
     assert abs(float(t.double().norm()) - 1.0) < 1e-5
 
 
+def test_scale_that_needs_a_gradient_is_refused():
+    table, ids = torch.ones(4, 8, device=DEV), torch.zeros(3, dtype=torch.long, device=DEV)
+    scale = torch.tensor(2.0, requires_grad=True)
+    with pytest.raises(TypeError, match="number"):
+        token_embedding(table, ids, scale=scale)
+    with torch.no_grad():
+        assert bool((token_embedding(table, ids, scale=scale) == 2).all())
+    assert bool((token_embedding(table, ids, scale=scale.detach()) == 2).all())
+
+
 @pytest.mark.parametrize("dim", [5, 72, 130, 1031])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_positions_outside_the_rows_are_neither_read_nor_written(dtype, dim):
