@@ -53,8 +53,12 @@ def clip_gradients(tensors, max_norm, *, out=None, eps=1e-6):
     """Scale ``tensors`` by ``min(1, max_norm / (norm + eps))``; returns the norm.
 
     In place, or into ``out`` (tensors of the same shapes and types); no output may share
-    memory with another tensor.  Autograd records neither the scaling nor the norm.  The norm is that before clipping; if it is NaN or infinite,
-    so are clipped values: ask ``isfinite`` of the norm to skip a step.
+    memory with another tensor.  Autograd records neither the scaling nor the norm.
+
+    The norm is that before clipping.  If it is NaN, so are all clipped values; an infinite value
+    makes the norm infinite, itself NaN and the finite values zero: ask ``isfinite`` of the norm to
+    skip a step.  The values are scaled by the norm in float64, so of finite values whose norm
+    passes float32 the clipped ones are right and only the returned norm is infinite.
     """
     what = "clip_gradients"
     tensors = _tensors(what, tensors)

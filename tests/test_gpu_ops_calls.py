@@ -133,6 +133,21 @@ def test_clipping_does_not_write_what_it_refuses():
     assert abs(float(t.double().norm()) - 1.0) < 1e-5
 
 
+def test_clipping_by_an_infinite_norm():
+    """As documented: finite values become zero, infinite ones NaN; a NaN norm makes all NaN."""
+    for bad, others in ((float("inf"), 0.0), (float("nan"), float("nan"))):
+        t = torch.ones(5000, device=DEV)
+        t[777] = bad
+        norm = clip_gradients([t], 1.0)
+        assert not bool(torch.isfinite(norm)) and bool(torch.isnan(t[777]))
+        t[777] = others
+        assert torch.equal(t.nan_to_num(7.0), torch.full_like(t, others).nan_to_num(7.0))
+    big = [torch.full((100,), 3e38, device=DEV) for _ in range(2)]  # beyond float32, not float64
+    norm = clip_gradients(big, 1.0)
+    assert bool(torch.isinf(norm))
+    assert all(abs(float(b.double().square().sum()) - 0.5) < 1e-5 for b in big)
+
+
 def test_scale_that_needs_a_gradient_is_refused():
     table, ids = torch.ones(4, 8, device=DEV), torch.zeros(3, dtype=torch.long, device=DEV)
     scale = torch.tensor(2.0, requires_grad=True)
