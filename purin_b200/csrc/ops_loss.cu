@@ -976,8 +976,23 @@ int32_t make_map(CUtensorMap* map, const void* base, int64_t columns, int64_t ro
   return r == CUDA_SUCCESS ? PURIN_OK : set_error(PURIN_ERR_CUDA, "loss: cuTensorMapEncodeTiled failed");
 }
 
+// CTA pairs that fit the device at once (a part of it with an odd number of SMs leaves one over).
+template <int kGroup>
+int groups_that_fit(void (*kernel)(Product), const cudaLaunchConfig_t& config, int device, int sms,
+                    std::atomic<int> (&known)[64]) {
+  const bool keeps = device >= 0 && device < 64;
+  int n = keeps ? known[device].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess || n <= 0) {
+    cudaGetLastError();  // not another call's error
+    return sms / kGroup;
+  }
+  if (keeps) known[device].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 template <typename T, int kGroup, Mode kMode>
-int32_t launch_product(const Product& p, int64_t most_items, int sms, cudaStream_t stream) {
+int32_t launch_product(const Product& p, int64_t most_items, int device, int sms, cudaStream_t stream) {
   using S = Shape<T, kGroup>;
   auto kernel = product_kernel<T, kGroup, kMode>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSharedBytes))
@@ -995,12 +1010,8 @@ int32_t launch_product(const Product& p, int64_t most_items, int sms, cudaStream
   config.attrs = attribute;
   config.numAttrs = p.row ? 2 : 1;  // without pack_rows_kernel it is the call's first
   if constexpr (kGroup > 1) {
-    // Pairs that fit the GPU at once (a part of it with an odd number of SMs leaves one over).
-    static const int fit = [&] {
-      int n = 0;
-      return cudaOccupancyMaxActiveClusters(&n, kernel, &config) == cudaSuccess && n > 0 ? n : sms / kGroup;
-    }();
-    sms = std::min(sms, fit * kGroup);
+    static std::atomic<int> known[64];  // of each device
+    sms = std::min(sms, groups_that_fit<kGroup>(kernel, config, device, sms, known) * kGroup);
   }
   config.gridDim = dim3(unsigned(std::min<int64_t>(most_items, sms / kGroup) * kGroup));
   return cuda_status(cudaLaunchKernelEx(&config, kernel, p));
@@ -1109,7 +1120,7 @@ int32_t forward(const PurinLossArgs* a, const Plan& p, char* ws, int sms, cudaSt
   q.stats = reinterpret_cast<float2*>(ws + p.stats);
   q.at_target = reinterpret_cast<float*>(ws + p.at_target);
   const int64_t items = ceil_div(a->tokens, kRows * kGroup) * p.groups;
-  if (int32_t bad = launch_product<T, kGroup, kStats>(q, items, sms, s)) return bad;
+  if (int32_t bad = launch_product<T, kGroup, kStats>(q, items, a->device, sms, s)) return bad;
   return cuda_status(launch_after(
       loss_kernel, dim3(unsigned(ceil_div(a->tokens, 32))), dim3(32 * kJoinGroups), 0, s, q.stats, q.at_target,
       int(p.groups) * Shape<T, kGroup>::kHalves,
@@ -1161,10 +1172,10 @@ int32_t backward(const PurinLossArgs* a, const Plan& p, char* ws, int sms, cudaS
       mapped = length;
     }
     const int64_t row_tiles = ceil_div(a->tokens, kRows * kGroup);
-    if (int32_t bad = launch_product<T, kGroup, kDz>(z, row_tiles * ceil_div(length, kColumns), sms, s)) return bad;
+    if (int32_t bad = launch_product<T, kGroup, kDz>(z, row_tiles * ceil_div(length, kColumns), a->device, sms, s)) return bad;
     const int64_t items = (q.want_hidden ? row_tiles * dim_tiles * p.splits : 0) +
                           (q.want_weight ? ceil_div(length, kRows * kGroup) * dim_tiles : 0);
-    if (int32_t bad = launch_product<T, kGroup, kProducts>(q, items, sms, s)) return bad;
+    if (int32_t bad = launch_product<T, kGroup, kProducts>(q, items, a->device, sms, s)) return bad;
   }
   const int64_t blocks = std::min<int64_t>(ceil_div(a->tokens * ceil_div(a->dim, 4), kPackThreads), int64_t(sms) * 16);
   const bool aligned = a->dim % 4 == 0 && reinterpret_cast<uintptr_t>(a->grad_hidden) % (4 * sizeof(T)) == 0;
