@@ -5,6 +5,7 @@
 #include <c10/core/InferenceMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
 #include <nvtx3/nvToolsExt.h>
@@ -53,26 +54,46 @@ void check(int32_t status, const char* name) {
   TORCH_CHECK(status == PURIN_OK, name, " failed (status ", status, "): ", purin_cp_last_error());
 }
 
+// Two events around one call, recorded on its stream.
+struct Recording {
+  Launch launch;
+  bool on;
+  cudaStream_t stream;
+  Recording(const char* name, int device, cudaStream_t s) : launch{name, nullptr, nullptr}, on(false), stream(s) {
+    if (!g_recording.load(std::memory_order_relaxed)) return;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    // A captured call runs at each replay: it has no time of its own.
+    on = cudaStreamIsCapturing(s, &capture) == cudaSuccess;
+    if (!on) cudaGetLastError();
+    on = on && capture == cudaStreamCaptureStatusNone;
+    if (!on) return;
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));  // the events are the stream's device's
+    on = cudaEventCreate(&launch.start) == cudaSuccess && cudaEventCreate(&launch.end) == cudaSuccess &&
+         cudaEventRecord(launch.start, s) == cudaSuccess;
+    if (!on) cudaGetLastError();  // not the call's error
+  }
+  void end() {
+    if (!on || cudaEventRecord(launch.end, stream) != cudaSuccess) return;
+    std::lock_guard<std::mutex> lock(g_launches_mutex);
+    g_launches.push_back(launch);
+    launch = {};
+  }
+  ~Recording() {
+    if (launch.start) cudaEventDestroy(launch.start);
+    if (launch.end) cudaEventDestroy(launch.end);
+  }
+};
+
 // Runs one entry point on the device's current stream in an NVTX range, between two events
 // while launches are recorded.
 template <typename F>
 void call(const char* name, int device, F&& f) {
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  Recording recording(name, device, stream);
   nvtxRangePushA(name);
-  Launch launch{name, nullptr, nullptr};
-  const bool record = g_recording.load(std::memory_order_relaxed);
-  if (record) {
-    cudaEventCreate(&launch.start);
-    cudaEventCreate(&launch.end);
-    cudaEventRecord(launch.start, stream);
-  }
   const int32_t status = f(static_cast<void*>(stream));
-  if (record) {
-    cudaEventRecord(launch.end, stream);
-    std::lock_guard<std::mutex> lock(g_launches_mutex);
-    g_launches.push_back(launch);
-  }
   nvtxRangePop();
+  recording.end();
   check(status, name);
 }
 
@@ -88,8 +109,8 @@ std::vector<std::pair<std::string, float>> recorded_launches() {
   std::vector<std::pair<std::string, float>> out;
   for (const Launch& l : launches) {
     float ms = 0.f;
-    cudaEventSynchronize(l.end);
-    cudaEventElapsedTime(&ms, l.start, l.end);
+    if (cudaEventSynchronize(l.end) != cudaSuccess || cudaEventElapsedTime(&ms, l.start, l.end) != cudaSuccess)
+      cudaGetLastError();
     cudaEventDestroy(l.start);
     cudaEventDestroy(l.end);
     out.emplace_back(l.name, ms);

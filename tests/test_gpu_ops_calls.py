@@ -211,3 +211,22 @@ def test_routings_that_are_not_whole_are_refused():
             dispatch_to_experts(x[:tokens], made)
         with pytest.raises(error):
             combine_from_experts(rows[:tokens * slots], weights[:tokens, :slots], made)
+
+
+def test_recording_leaves_captured_calls_out():
+    """A captured call has no time of its own; asking for it is not the next call's error."""
+    from purin_b200 import _native_ops
+
+    x, ids = torch.ones(5, 4, device=DEV), torch.zeros(3, dtype=torch.long, device=DEV)
+    token_embedding(x, ids)
+    torch.cuda.synchronize()
+    _native_ops.recorded_launches()
+    _native_ops.record_launches(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = token_embedding(x, ids)
+    gradient_norm(x)
+    _native_ops.record_launches(False)
+    assert [name for name, ms in _native_ops.recorded_launches() if ms > 0] == ["purin_gradients"]
+    graph.replay()
+    assert torch.equal(captured, token_embedding(x, ids))
