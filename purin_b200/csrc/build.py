@@ -29,6 +29,7 @@ OPS_SOURCES = ["ops_sort.cu", "ops_embedding.cu", "ops_routing.cu", "ops_loss.cu
                "ops_gradients.cu"]
 TORCH_SOURCE = "ops_torch.cpp"
 TORCH_LIB = LIB_DIR / "_ops_torch.so"
+TORCH_STAMP = LIB_DIR / "_ops_torch.built_for"  # the torch and CPython that it was compiled against
 # cp_forward.cu is also compiled once per (dtype, shared values, QP) combination
 # of its kernels, so that the heavy template instantiations build in parallel.
 FORWARD_PARTS = [(t, sh, qp) for t in ("double", "float") for sh in ("true", "false")
@@ -58,8 +59,19 @@ def _inputs():
     return files
 
 
+def built_for() -> str:
+    """What the binding depends on besides its sources: torch's and CPython's binary interfaces."""
+    import sysconfig
+
+    import torch
+
+    return f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}\n"
+
+
 def up_to_date() -> bool:
-    if not LIB.exists() or not TORCH_LIB.exists():
+    if not LIB.exists() or not TORCH_LIB.exists() or not TORCH_STAMP.exists():
+        return False
+    if TORCH_STAMP.read_text() != built_for():
         return False
     stamp = min(LIB.stat().st_mtime, TORCH_LIB.stat().st_mtime)
     return all(f.stat().st_mtime <= stamp for f in _inputs())
@@ -98,6 +110,7 @@ def _link_torch(obj: str):
         sys.stderr.write(proc.stdout + proc.stderr)
         raise RuntimeError("g++ failed linking _ops_torch.so")
     os.replace(tmp, TORCH_LIB)
+    TORCH_STAMP.write_text(built_for())
 
 
 def build(verbose: bool = False, force: bool = False) -> Path:
