@@ -9,14 +9,24 @@
 //   products  dh += dz W and dW = dz^T h of that piece, in one launch: their tiles fill the
 //             SMs' last round together
 // The piece of dz is the only thing of the size tokens x vocabulary that ever exists, and it
-// is bounded (kPieceBytes); making z twice costs a quarter of the whole step's products.
+// is bounded: kPieceBytes, or kLeastColumns of every token where those are more.  Making z twice
+// costs a quarter of the whole step's products.
 //
 // Only tokens with a target take part: pack_rows_kernel moves their rows to the front (in order)
 // and the others behind them as zeros, so an ignored token costs nothing and whatever its
 // row holds reaches no gradient.  It also gives every row the alignment that TMA needs.
 //
+// Bits.  bfloat16: the sums of a product stay in the tensor cores over all of K, in 32 bits, but
+// their adder truncates: each 16 of K drop up to 2^-23 of the sum so far, and logits come out a little
+// small (the losses of 4096 x 32768 x 1024 and 8192 x 131072 x 2048 are off by 3.3e-7 and 5.6e-7 of
+// themselves, by 2e-8 and less with products in float32).  The operands' own rounding is 2^-9.
+// dz is rounded to bfloat16 for its two products, whose operands have one type: the rounding
+// differs from element to element and the sums average it, so gradients move by 3 to 6.4e-4, and
+// their error against 64 bits stays what their own rounding to bfloat16 makes it (1.67e-3, against
+// 1.66e-3 with dz in 32 bits).  More bits would be a second part of dz, and twice the products.
+//
 // float32: a value is the exact sum of three bfloat16 parts, and the six products of parts
-// that matter (the rest is below 2^-23 of |a||b|) go into one accumulator.
+// that matter (the rest is below 2^-22 of |a||b|) go into one accumulator.
 #include <algorithm>
 
 #include "ops_common.cuh"
@@ -34,6 +44,7 @@ constexpr int kGroupRows = 4096;      // rows whose tiles run together (their sh
 // Piece of dz: smaller ones fit L2 better but make dh's sums be read and written more often
 // (backward of 8192 x 131072 x 2048: 64 MB 11.0 ms, 128 MB 10.4, 256 MB 10.2, 512 MB 10.15).
 constexpr size_t kPieceBytes = size_t(256) << 20;
+constexpr int64_t kLeastColumns = 1024;  // of a piece, more bytes or not: 131072 tokens and up in bfloat16
 constexpr size_t kStatsBytes = size_t(256) << 20;
 constexpr float kLog2E = 1.4426950408889634f;
 
@@ -652,7 +663,8 @@ struct PackRows {
 };
 
 // Block b places tokens [b per_block, (b + 1) per_block).  Every block counts the targets of
-// all tokens itself: 8 bytes a token, against the 2 dim bytes a token that are packed.
+// all tokens itself: 8 bytes a token and block, from L2.  At 8192 tokens the 1024 blocks read 64 KB
+// each and pack 32 KB of dim 2048; beyond 16384 tokens there are 2048 blocks, however many tokens.
 template <typename T>
 __global__ void __launch_bounds__(kPackThreads) pack_rows_kernel(PackRows a, Targets y) {
   constexpr int kWarps = kPackThreads / 32;
@@ -928,9 +940,9 @@ Plan plan_of(const PurinLossArgs* a, bool backward, int sms) {
     p.stats = take(size_t(p.groups) * halves * n * 8);
     p.at_target = take(n * 4);
   } else {
-    // As many columns of dz as kPieceBytes hold, at least 1024, in pieces of about one size.
+    // As many columns of dz as kPieceBytes hold, at least kLeastColumns, in pieces of about one size.
     int64_t most = int64_t(kPieceBytes / (2 * p.parts) / std::max<size_t>(n, 1)) / kColumns;
-    most = std::min(std::max<int64_t>(most, 1024 / kColumns), columns);
+    most = std::min(std::max<int64_t>(most, kLeastColumns / kColumns), columns);
     p.piece = ceil_div(columns, ceil_div(columns, most)) * kColumns;
     p.dz = take(p.parts * n * p.piece * 2);
     p.sum_pitch = ceil_div(a->dim, 32) * 32;
