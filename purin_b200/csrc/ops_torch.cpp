@@ -9,12 +9,14 @@
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
 #include <nvtx3/nvToolsExt.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <atomic>
 #include <mutex>
+#include <optional>
 #include <string>
 #include <tuple>
 #include <utility>
@@ -272,6 +274,25 @@ std::tuple<Tensor, Tensor, Tensor> route(const Tensor& given, int64_t num_expert
   return {offsets, position, source};
 }
 
+// A routing that a kernel may read, whole and on x's device.  `source` may be undefined.
+void check_routing(const std::string& what, const Tensor& x, const Tensor& offsets, const Tensor& position,
+                   const std::optional<Tensor>& source) {
+  TORCH_CHECK_VALUE(position.dim() == 2 && position.size(1) >= 1 && offsets.dim() == 1 && offsets.size(0) >= 2, what,
+                    ": the routing's position must have shape (tokens, slots) and offsets (experts + 1,), got ",
+                    position.sizes(), " and ", offsets.sizes());
+  TORCH_CHECK_TYPE(position.scalar_type() == at::kInt && offsets.scalar_type() == at::kInt, what,
+                   ": the routing's position and offsets must be int32, got ", position.scalar_type(), " and ",
+                   offsets.scalar_type());
+  TORCH_CHECK_VALUE(position.is_contiguous() && offsets.is_contiguous(), what,
+                    ": the routing's position and offsets must be contiguous, as route_to_experts makes them");
+  // Positions name rows of the whole routing: of a part of it, rows that are not there.
+  TORCH_CHECK_VALUE(!source || source->numel() == position.numel(), what, ": the routing has ", source->numel(),
+                    " slots but ", position.numel(), " positions");
+  TORCH_CHECK(x.is_cuda(), what, " runs on CUDA devices only; got a tensor on ", x.device());
+  TORCH_CHECK_VALUE(position.device() == x.device() && offsets.device() == x.device(), what, ": tensors are on ",
+                    x.device(), ", ", position.device(), " and ", offsets.device());
+}
+
 PurinRouteRowsArgs rows_args(const Tensor& rows, const Tensor& offsets, const Tensor& position) {
   PurinRouteRowsArgs a = {};
   a.device = rows.get_device();
@@ -477,12 +498,13 @@ Tensor gradients(const std::vector<Tensor>& tensors, const std::vector<Tensor>& 
                  double max_norm, double eps) {
   const char* what = clip ? "clip_gradients" : "gradient_norm";
   refuse_tracing(what);
+  const bool forward_mode = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
   std::vector<PurinGradient> list(tensors.size());
   bool wide = false, graph = false;
   for (size_t i = 0; i < tensors.size(); ++i) {
-    refuse_tangent(what, tensors[i]);
+    if (forward_mode) refuse_tangent(what, tensors[i]);
     if (clip) {
-      refuse_tangent(what, outs[i]);
+      if (forward_mode) refuse_tangent(what, outs[i]);
       // Counting the change below would raise, behind a launch that has written.
       TORCH_CHECK(!outs[i].is_inference() || c10::InferenceMode::is_enabled(), what,
                   ": a tensor of inference mode is not written outside it");
@@ -518,6 +540,7 @@ Tensor gradients(const std::vector<Tensor>& tensors, const std::vector<Tensor>& 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding", &embedding);
   m.def("route", &route);
+  m.def("check_routing", &check_routing);
   m.def("dispatch", &dispatch);
   m.def("combine", &combine);
   m.def("linear_cross_entropy", &linear_cross_entropy);

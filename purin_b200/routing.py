@@ -54,20 +54,9 @@ def route_to_experts(experts, num_experts) -> ExpertRouting:
 
 
 def _check_routing(what, x, routing):
-    """``x`` and the routing are on one CUDA device, and the routing is whole."""
+    """The routing is whole, and on the CUDA device of ``x``."""
     offsets, position, source = routing
-    _ops.require_cuda(what, x, position, offsets)
-    if position.dim() != 2 or position.shape[1] < 1 or offsets.dim() != 1 or offsets.shape[0] < 2:
-        raise ValueError(f"{what}: the routing's position must have shape (tokens, slots) and offsets "
-                         f"(experts + 1,), got {tuple(position.shape)} and {tuple(offsets.shape)}")
-    for name, t in (("position", position), ("offsets", offsets)):
-        if t.dtype != torch.int32:
-            raise TypeError(f"{what}: the routing's {name} must be int32, got {t.dtype}")
-        if not t.is_contiguous():
-            raise ValueError(f"{what}: the routing's {name} must be contiguous; route_to_experts makes it so")
-    # Positions name rows of the whole routing: of a part of it, rows that are not there.
-    if isinstance(source, torch.Tensor) and source.numel() != position.numel():
-        raise ValueError(f"{what}: the routing has {source.numel()} slots but {position.numel()} positions")
+    _ops.load().check_routing(what, x, offsets, position, source)
 
 
 def _check_rows(what, name, t, rows):

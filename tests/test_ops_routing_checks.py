@@ -12,16 +12,17 @@ def whole(tokens=4, slots=2, experts=3):
                          torch.arange(n, dtype=torch.int32).view(tokens, slots), torch.arange(n, dtype=torch.int32))
 
 
-@pytest.fixture(autouse=True)
-def any_device(monkeypatch):
-    """The checks behind that of the device."""
-    monkeypatch.setattr(routing._ops, "require_cuda", lambda what, *tensors: None)
+@pytest.fixture(autouse=True, scope="module")
+def built():
+    from purin_b200.csrc.build import build
+
+    build()
 
 
-def test_a_whole_routing_passes():
-    routing._check_routing("dispatch", torch.zeros(4, 8), whole())
-    routing._check_routing("dispatch", torch.zeros(4, 8), whole()._replace(source=None))
-    routing._check_routing("dispatch", torch.zeros(0, 8), whole(tokens=0))
+def test_a_whole_routing_passes_up_to_the_device():
+    for made, tokens in ((whole(), 4), (whole()._replace(source=None), 4), (whole(tokens=0), 0)):
+        with pytest.raises(RuntimeError, match="CUDA devices only"):
+            routing._check_routing("dispatch", torch.zeros(tokens, 8), made)
 
 
 @pytest.mark.parametrize("error,change", [
