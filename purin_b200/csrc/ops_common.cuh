@@ -77,6 +77,12 @@ inline int sm_count(int device) {
   return n;
 }
 
+// Blocks of a kernel that goes round its items: one round, of 32 blocks an SM at most.
+inline unsigned grid_for(int64_t items, int64_t per_block, int sms) {
+  const int64_t blocks = ceil_div(items, per_block), most = int64_t(sms) * 32;
+  return unsigned(blocks < most ? (blocks > 0 ? blocks : 1) : most);
+}
+
 // Sums and products are held in 32 bits, in 64 for double.
 template <typename T> struct Accumulator { using type = float; };
 template <> struct Accumulator<double> { using type = double; };

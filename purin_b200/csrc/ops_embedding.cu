@@ -240,11 +240,6 @@ BackwardLayout backward_layout(const PurinEmbeddingArgs* a) {
   return l;
 }
 
-unsigned grid_for(int64_t items, int64_t per_block, int sms) {
-  const int64_t blocks = ceil_div(items, per_block), most = int64_t(sms) * 32;
-  return unsigned(blocks < most ? (blocks > 0 ? blocks : 1) : most);
-}
-
 }  // namespace
 }  // namespace ops
 }  // namespace purin

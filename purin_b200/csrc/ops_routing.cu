@@ -216,11 +216,6 @@ combine_backward_kernel(const int32_t* position, const int32_t* kept_rows, int64
   }
 }
 
-unsigned grid_for(int64_t items, int64_t per_block, int sms) {
-  const int64_t blocks = ceil_div(items, per_block), most = int64_t(sms) * 32;
-  return unsigned(blocks < most ? (blocks > 0 ? blocks : 1) : most);
-}
-
 int32_t check_route(const PurinRouteArgs* a) {
   if (!a) return invalid("route: null arguments");
   if (a->tokens < 0 || a->slots < 1 || a->num_experts < 1) return invalid("route: invalid sizes");
