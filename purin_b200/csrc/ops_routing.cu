@@ -52,18 +52,15 @@ spread_kernel(const int32_t* position, const int32_t* kept_rows, int64_t tokens,
       if (C == 1 || c + j * items < packs) p[j] = *reinterpret_cast<const Pack<T, V>*>(x + t * stride + (c + j * items) * V);
 #pragma unroll
     for (int i = 0; i < V; ++i) zero.v[i] = narrow<T>(acc_t<T>(0));
-    constexpr int kAhead = 4;  // positions loaded at a time
-    for (int first = 0; first < slots; first += kAhead) {
-      int32_t r[kAhead];
+#pragma unroll 4
+    for (int k = 0; k < slots; ++k) {
+      const int32_t r = position[t * slots + k];
+      const bool inside = below(r, rows);
+      Pack<T, V>* to = reinterpret_cast<Pack<T, V>*>(out) + int64_t(r) * packs + c;
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) r[k] = first + k < slots ? position[t * slots + first + k] : -1;
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        if (!below(r[k], rows)) continue;
-        Pack<T, V>* to = reinterpret_cast<Pack<T, V>*>(out) + r[k] * packs + c;
-#pragma unroll
-        for (int j = 0; j < C; ++j)
-          if (C == 1 || c + j * items < packs) to[j * items] = r[k] < kept ? p[j] : zero;
+      for (int j = 0; j < C; ++j) {
+        const Pack<T, V> q = r < kept ? p[j] : zero;
+        if (inside && (C == 1 || c + j * items < packs)) to[j * items] = q;
       }
     }
   }
