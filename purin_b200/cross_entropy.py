@@ -24,10 +24,11 @@ def linear_cross_entropy(hidden, weight, targets, *, ignore_index=-100, reductio
     that count; 0 if none does), "sum" or "none".  Differentiable in ``hidden`` and ``weight``;
     the logits are not kept, the backward makes them again.  bfloat16 products are exact and
     summed in float32 by an adder that truncates (a mean loss is off by some 5e-7 of itself), and the
-    logits' gradient is rounded to bfloat16 before its products; float32 operands keep float32
-    accuracy and have to be finite (the parts of an infinite one can make its logits NaN).  Should a kernel's bounded wait run out, every loss or gradient of the call is NaN.
+    logits' gradient is rounded to bfloat16 before its products.  float32 operands keep float32
+    accuracy, and have to be finite: the parts of an infinite one can make its logits NaN.
     Beside its outputs a backward holds 256 MB of the logits' gradient at most, or 1024 columns of it
-    where those are more (2 bytes a value for bfloat16, 6 for float32).
+    where those are more (2 bytes a value for bfloat16, 6 for float32).  Should a kernel's bounded
+    wait run out, every loss or gradient of the call is NaN.
     """
     _ops.require_cuda(_WHAT, hidden, weight, targets)
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1] \
